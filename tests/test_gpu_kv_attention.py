@@ -325,6 +325,31 @@ def test_binding_refuses_short_tensors(ctx):
         N.KvBatch(s.dtable, s.dstarts[:1], s.dlen, 3, 3, 20)
 
 
+def test_binding_refuses_values_of_another_type(ctx):
+    """fp32 queries (what ns_qkv leaves), an output of the other type, fp64 frequencies and bf16 are refused by the calls."""
+    s = Setup(F16, 64, 4, 2, 16, [(3, 20)], seed=68)
+    q = s.queries().cuda()
+    for bad in (q.float(), q.bfloat16()):
+        with pytest.raises(TypeError, match="float16"):
+            s.attend(ctx, bad)
+        with pytest.raises(TypeError, match="float16"):
+            s.attend(ctx, bad, prefix=0)
+    with pytest.raises(TypeError, match="float16"):
+        s.attend(ctx, q, out=torch.empty(3, 4, 64, device="cuda"))
+    with pytest.raises(TypeError, match="float32"):
+        s.attend(ctx, q, half_out=False, out=torch.empty(6, 4, 64, dtype=F16, device="cuda"))
+    x = [torch.randn(3, h, 64, device="cuda") for h in (4, 2, 2)]
+    freqs, before = torch.ones(32, device="cuda"), s.dk.clone()
+    for i, bad in ((0, x[0].double()), (1, torch.zeros(12, 2, 64, dtype=F16, device="cuda"))):
+        with pytest.raises(TypeError, match="float32"):
+            ctx.kv_append(s.cache, s.batch, *x[:i], bad, *x[i + 1:], 4, freqs, 64, q)
+    with pytest.raises(TypeError, match="float32"):
+        ctx.kv_append(s.cache, s.batch, *x, 4, freqs.double(), 64, q)
+    with pytest.raises(TypeError, match="float16"):
+        ctx.kv_append(s.cache, s.batch, *x, 4, freqs, 64, q.float())
+    assert torch.equal(s.dk, before)
+
+
 @pytest.mark.parametrize("many", [False, True], ids=["few-rows", "tiles"])
 def test_contradicting_sequences_and_pages_are_nan(ctx, many):
     n = 20 if many else 2
