@@ -12,7 +12,7 @@
 // the consecutive ones which the same lane feeds back as the P^T operand of the second product: P
 // never leaves its lane, and the statistics of a row need one or two lane exchanges.
 //
-// Work that is split over the keys leaves parts (O unnormalised, m in powers of two, l) in the
+// Work that is split over the keys leaves parts (O unnormalised, m as a score before the scale, l) in the
 // workspace.  Parts are joined in part order, so results do not depend on the order of arrival, by the last
 // workgroup of a sequence and key head to arrive (few rows) or by a launch of its own (tiles).  No
 // workgroup waits for another.
@@ -40,6 +40,19 @@ template <bool HILO>
 constexpr float kBias = HILO ? 14.0f : 9.0f;
 template <bool HILO>
 constexpr float kLag = HILO ? 1.5f : 6.0f;
+template <bool HILO>
+constexpr float kUnbias = HILO ? 0x1p-14f : 0x1p-9f;  // parts are kept without the bias: both kinds may meet in a join
+// P = 2^(c1 s - (c1 m - bias)) is one operation a score.  What is in brackets is rounded, by 2^-15 while c1 |m| is at most
+// kFar; far above it the rounding would move P by whole powers of two (past 65504, or to nothing).  There s - m is
+// formed first, exact for the scores that weigh: a wave with such a row, or with one that has seen nothing yet (m = -inf, its
+// scores as well: 0 is subtracted), takes the branch of a raised maximum for every tile.  Parts are compared by m
+// itself for the same reason.  (2,048 tokens at 32,768 keys 1,028 -> 1,034 us, 157 tokens 22.4 -> 22.7, against always the
+// one operation.)
+constexpr float kFar = 1024.0f;
+// The |m| from which a row is far.  Formed in the kernel: a launch argument more costs each of them some .2 us.
+__device__ __forceinline__ float far_max(float c1) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, kFar * __builtin_amdgcn_rcpf(c1))));
+}
 constexpr uint32_t kRowsMax = 16;  // rows of a sequence and key head up to which the few-row kernel takes them
 
 struct AttnArgs {
@@ -152,13 +165,13 @@ __device__ void join_rows(const AttnArgs &a, const Parts &ps, uint32_t rows, uin
 #pragma unroll
             for (int u = 0; u < B; ++u) top = __builtin_fmaxf(top, st[u].x);
             const float zero = top == -__builtin_inff() ? 0.f : top;  // parts that see nothing of this row
-            const float f = exp2f_fast(M - zero);
+            const float f = exp2f_fast((M - zero) * a.c1);
             M = top;
             l *= f;
             o = float4{o.x * f, o.y * f, o.z * f, o.w * f};
 #pragma unroll
             for (int u = 0; u < B; ++u) {
-                const float w = exp2f_fast(st[u].x - zero);
+                const float w = exp2f_fast((st[u].x - zero) * a.c1);
                 l = __builtin_fmaf(w, st[u].y, l);
                 o.x = __builtin_fmaf(w, x[u].x, o.x);
                 o.y = __builtin_fmaf(w, x[u].y, o.y);
@@ -184,7 +197,7 @@ __device__ void join_rows(const AttnArgs &a, const Parts &ps, uint32_t rows, uin
         for (uint32_t i = 0; i < ng; ++i) {
             const float2 s = red_ml[i * rows + r];
             const float4 x = red[i * cols + tid];
-            const float w = exp2f_fast(s.x - M);
+            const float w = exp2f_fast((s.x - M) * a.c1);
             l = __builtin_fmaf(w, s.y, l);
             o = float4{__builtin_fmaf(w, x.x, o.x), __builtin_fmaf(w, x.y, o.y), __builtin_fmaf(w, x.z, o.z), __builtin_fmaf(w, x.w, o.w)};
         }
@@ -215,12 +228,12 @@ __device__ __forceinline__ void join_row(const AttnArgs &a, const Parts &ps, uin
 #pragma unroll
         for (int u = 0; u < 8; ++u) top = __builtin_fmaxf(top, st[u].x);
         if (top == -__builtin_inff()) top = 0.f;  // parts that see nothing of this row
-        const float f = exp2f_fast(M - top);
+        const float f = exp2f_fast((M - top) * a.c1);
         l *= f;
         o = float4{o.x * f, o.y * f, o.z * f, o.w * f};
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-            const float w = exp2f_fast(st[u].x - top);
+            const float w = exp2f_fast((st[u].x - top) * a.c1);
             l = __builtin_fmaf(w, st[u].y, l);
             o.x = __builtin_fmaf(w, x[u].x, o.x);
             o.y = __builtin_fmaf(w, x[u].y, o.y);
@@ -384,6 +397,7 @@ __device__ __forceinline__ void attn_rows(const AttnArgs &a, uint32_t block) {
     float4_t o[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[d] = float4_t{0.f, 0.f, 0.f, 0.f};
+    const float far_m = far_max(a.c1);
     float m = -__builtin_inff(), l = 0.f;
     u32x4 kf[NT][JS], vf[DT];
 
@@ -494,15 +508,24 @@ __device__ __forceinline__ void attn_rows(const AttnArgs &a, uint32_t block) {
         top = __builtin_fmaxf(top, __shfl_xor(top, 16));
         top = __builtin_fmaxf(top, __shfl_xor(top, 32));
         const float mn = __builtin_fmaxf(m, top);
-        if (__ballot((mn - m) * a.c1 > kLag<true>)) {  // some row's maximum left the lag (from -inf: infinitely)
+        bool far = false;
+        if (__ballot((mn - m) * a.c1 > kLag<true> || __builtin_fabsf(m) > far_m)) {  // some row's maximum left the lag (from -inf: infinitely)
             const float f = mn == m ? 1.f : exp2f_fast((m - mn) * a.c1);
             l *= f;
 #pragma unroll
             for (int d = 0; d < DT; ++d) o[d] *= f;
             m = mn;
+            if (__ballot(__builtin_fabsf(m) > far_m)) {
+                const float zero = m == -__builtin_inff() ? 0.f : m;
+#pragma unroll
+                for (int i = 0; i < NT; ++i) {
+                    keep_branch(sc[i]);
+                    sc[i] -= zero;
+                }
+                far = true;
+            }
         }
-        // A row that has seen nothing yet keeps m = -inf: its scores are -inf as well, and 0 is subtracted.
-        const float mc = m == -__builtin_inff() ? 0.f : m * a.c1 - kBias<true>;
+        const float mc = far ? -kBias<true> : __builtin_fmaf(m, a.c1, -kBias<true>);
         half8_t hi[U], lw[U];
 #pragma unroll
         for (int i = 0; i < NT; ++i)
@@ -550,7 +573,7 @@ __device__ __forceinline__ void attn_rows(const AttnArgs &a, uint32_t block) {
     // ---- the waves' parts: common maximum, then the sum in wave order
     const uint32_t pitch = D + 4;
     if (g == 0) {
-        wm[wave][col] = m * a.c1 - kBias<true>;  // -inf stays -inf: c1 > 0
+        wm[wave][col] = m;
         wl[wave][col] = l;
     }
     if (col < rows) {
@@ -569,7 +592,7 @@ __device__ __forceinline__ void attn_rows(const AttnArgs &a, uint32_t block) {
         float4 acc{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            const float f = M == -__builtin_inff() ? 1.f : exp2f_fast(wm[w][r] - M);
+            const float f = M == -__builtin_inff() ? 1.f : exp2f_fast(__builtin_fmaf(wm[w][r] - M, a.c1, -kBias<true>));
             const float4_t x = *reinterpret_cast<const float4_t *>(&lds[(w * a.row_cap + r) * pitch + d]);
             L = __builtin_fmaf(f, wl[w][r], L);
             acc.x = __builtin_fmaf(f, x[0], acc.x);
@@ -801,6 +824,7 @@ __device__ __forceinline__ void attn_mid(const AttnArgs &a, uint32_t block, uint
     float16_t o[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[d] = float16_t{};
+    const float far_m = far_max(a.c1);
     float m = -__builtin_inff(), l = 0.f;
     for (; tile < end; tile += 4) {
         load_v(tile);
@@ -830,14 +854,21 @@ __device__ __forceinline__ void attn_mid(const AttnArgs &a, uint32_t block, uint
         for (int v = 1; v < 16; ++v) top = __builtin_fmaxf(top, sc[v]);
         top = max_halves(top);
         const float mn = __builtin_fmaxf(m, top);
-        if (__ballot((mn - m) * a.c1 > kLag<HILO>)) {
+        bool far = false;
+        if (__ballot((mn - m) * a.c1 > kLag<HILO> || __builtin_fabsf(m) > far_m)) {
             const float f = mn == m ? 1.f : exp2f_fast((m - mn) * a.c1);
             l *= f;
 #pragma unroll
             for (int d = 0; d < DT; ++d) o[d] *= f;
             m = mn;
+            if (__ballot(__builtin_fabsf(m) > far_m)) {
+                const float zero = m == -__builtin_inff() ? 0.f : m;
+                keep_branch(sc);
+                sc -= zero;
+                far = true;
+            }
         }
-        const float mc = m == -__builtin_inff() ? 0.f : m * a.c1 - kBias<HILO>;
+        const float mc = far ? -kBias<HILO> : __builtin_fmaf(m, a.c1, -kBias<HILO>);
         half8_t ph[2], pl[2];
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
@@ -884,7 +915,7 @@ __device__ __forceinline__ void attn_mid(const AttnArgs &a, uint32_t block, uint
 
     const uint32_t pitch = D + 4;
     if (hl == 0) {
-        wm[wave][col] = m * a.c1 - kBias<HILO>;
+        wm[wave][col] = m;
         wl[wave][col] = l;
     }
     if (col < rows) {
@@ -906,7 +937,7 @@ __device__ __forceinline__ void attn_mid(const AttnArgs &a, uint32_t block, uint
         float4 acc{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            const float f = M == -__builtin_inff() ? 1.f : exp2f_fast(wm[w][r] - M);
+            const float f = M == -__builtin_inff() ? 1.f : exp2f_fast(__builtin_fmaf(wm[w][r] - M, a.c1, -kBias<HILO>));
             const float4_t x = *reinterpret_cast<const float4_t *>(&lds[(w * TM + r) * pitch + d]);
             L = __builtin_fmaf(f, wl[w][r], L);
             acc.x = __builtin_fmaf(f, x[0], acc.x);
@@ -989,6 +1020,7 @@ __device__ __forceinline__ void attn_tile(const AttnArgs &a, uint32_t block, uin
     float16_t o[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[d] = float16_t{};
+    const float far_m = far_max(a.c1);
     float m = -__builtin_inff(), l = 0.f;
     bool bad = false;
 
@@ -1112,14 +1144,21 @@ __device__ __forceinline__ void attn_tile(const AttnArgs &a, uint32_t block, uin
         for (int v = 1; v < 16; ++v) top = __builtin_fmaxf(top, sc[v]);
         top = max_halves(top);
         const float mn = __builtin_fmaxf(m, top);
-        if (__ballot((mn - m) * a.c1 > kLag<HILO>)) {
+        bool far = false;
+        if (__ballot((mn - m) * a.c1 > kLag<HILO> || __builtin_fabsf(m) > far_m)) {
             const float f = mn == m ? 1.f : exp2f_fast((m - mn) * a.c1);
             l *= f;
 #pragma unroll
             for (int d = 0; d < DT; ++d) o[d] *= f;
             m = mn;
+            if (__ballot(__builtin_fabsf(m) > far_m)) {
+                const float zero = m == -__builtin_inff() ? 0.f : m;
+                keep_branch(sc);
+                sc -= zero;
+                far = true;
+            }
         }
-        const float mc = m == -__builtin_inff() ? 0.f : m * a.c1 - kBias<HILO>;
+        const float mc = far ? -kBias<HILO> : __builtin_fmaf(m, a.c1, -kBias<HILO>);
         half8_t ph[2], pl[2];
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
@@ -1150,7 +1189,7 @@ __device__ __forceinline__ void attn_tile(const AttnArgs &a, uint32_t block, uin
     const uint64_t own_step = uint64_t(a.kv.kv_heads) * (PREFIX ? a.pre_rows : TM);
     const uint64_t own_row = PREFIX ? a.pre_row + uint64_t(head) * a.pre_rows + row0 : (uint64_t(slot) * n_parts * a.kv.kv_heads + head) * TM;
     if (!mine) return;
-    const float f = whole ? a.v_scale / l : 1.f;
+    const float f = whole ? a.v_scale / l : kUnbias<HILO>;
     const uint64_t at = own_row + part * own_step + (wrow - row0) + col;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -1161,7 +1200,7 @@ __device__ __forceinline__ void attn_tile(const AttnArgs &a, uint32_t block, uin
             if (whole) write_out<D>(a, token, qhead, dim, v);
             else *reinterpret_cast<float4 *>(a.rows + at * D + dim) = v;
         }
-    if (!whole && hl == 0) *reinterpret_cast<float2 *>(a.stats + 2 * at) = float2{m * a.c1 - kBias<HILO>, l};
+    if (!whole && hl == 0) *reinterpret_cast<float2 *>(a.stats + 2 * at) = float2{m, l * kUnbias<HILO>};
 }
 template <int D, bool E4M3, int NW, int NS>
 struct TileLds {

@@ -712,7 +712,7 @@ int attention(ns_ctx *ctx, const char *fn, const ns_kv_cache *c, const ns_kv_bat
     KvArgs kv;
     if (int rc = check_kv(ctx, fn, c, b, q_heads, &kv)) return rc;
     if (!q || !out || !aligned16(q) || !aligned16(out)) return bad(NS_ERR_ARG, "q and out must be non-null and 16-byte aligned");
-    // 1e-30 and 1e30: the factor of the scores and its products with fp16 queries stay inside fp32
+    // 1e-30 and 1e30: the scores' factor, with log2(e), is a normal fp32 (their products with it need not be finite)
     if (!(scale > 0.f) || !std::isfinite(scale) || !(scale * c->k_scale > 1e-30f) || !(scale * c->k_scale < 1e30f))
         return bad(NS_ERR_ARG, "scale must be positive and finite, and its product with k_scale between 1e-30 and 1e30");
     const uint64_t prefix = uint64_t(prefix_pages) * c->page_size;
