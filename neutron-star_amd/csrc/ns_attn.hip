@@ -227,13 +227,13 @@ __device__ __forceinline__ void join_row(const AttnArgs &a, const Parts &ps, uin
         float top = M;
 #pragma unroll
         for (int u = 0; u < 8; ++u) top = __builtin_fmaxf(top, st[u].x);
-        if (top == -__builtin_inff()) top = 0.f;  // parts that see nothing of this row
-        const float f = exp2f_fast((M - top) * a.c1);
+        const float zero = top == -__builtin_inff() ? 0.f : top;  // parts that see nothing of this row: M stays -inf
+        const float f = exp2f_fast((M - zero) * a.c1);
         l *= f;
         o = float4{o.x * f, o.y * f, o.z * f, o.w * f};
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-            const float w = exp2f_fast((st[u].x - top) * a.c1);
+            const float w = exp2f_fast((st[u].x - zero) * a.c1);
             l = __builtin_fmaf(w, st[u].y, l);
             o.x = __builtin_fmaf(w, x[u].x, o.x);
             o.y = __builtin_fmaf(w, x[u].y, o.y);

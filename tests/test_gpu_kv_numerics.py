@@ -1,5 +1,5 @@
 """GPU tests of where attention's arithmetic could go wrong, against the 64-bit oracle with scores that fp32 holds exactly:
-scores of any size."""
+scores of any size, and of minus infinity."""
 import math
 
 import pytest
@@ -88,3 +88,30 @@ def test_scores_of_any_size(ctx, tiles, case, top, half_out):
         assert_within(got, ref, bound + slack * float(s.vs * s.v.float().abs().max()))
         if s.max_q * (qh // kh) <= 16 and prefix is None:
             break
+
+
+@pytest.mark.parametrize("mid", [0, 1], ids=["128", "32"])
+@pytest.mark.parametrize("prefix", [None, 20])
+def test_parts_that_see_only_minus_infinity(ctx, tiles, mid, prefix):
+    """Keys of minus infinity weigh nothing; a row whose first parts hold nothing else is the rest's, however low the
+    rest's scores are."""
+    D, page, n = 64, 16, (20 if prefix is None else 1)
+    lengths = [(n, 400)] if prefix is None else [(1, 330), (1, 325)]
+    s = Setup(F16, D, 4, 2, page, lengths, seed=230 + mid, shared=prefix or 0)
+    k = torch.zeros(s.k.shape)
+    k[:, :, 0, :, 0] = -math.inf
+    seen = [(int(s.table[0, p // page]), p % page) for p in (range(300, 380) if prefix is None else range(290, 320))]
+    for pg, slot in seen:
+        k[pg, :, 0, slot, 0] = 0
+        k[pg, :, 0, slot, 1] = -2048.0
+    s.k = k.half()
+    s.device()
+    q = torch.zeros(s.rows, 4, D)
+    q[..., 0], q[..., 1] = 1.0, 2.0  # scores -512: 2^-738 against zero
+    q = q.half()
+    tiles(mid, 32)
+    got = attend(ctx, s, q, 0.125, True, prefix).double().cpu()
+    pages, slot = torch.tensor([x[0] for x in seen]), torch.tensor([x[1] for x in seen])
+    v = s.v.double()[pages, :, slot // 8, :, slot % 8]  # [keys][kv heads][D]
+    ref = v.mean(0).repeat_interleave(2, 0)[None].expand(s.T, 4, D)
+    assert_within(got, ref, (2 * O.U16 + 2.0 ** -14) * v.abs().mean(0).repeat_interleave(2, 0)[None] + 2.0 ** -24)
