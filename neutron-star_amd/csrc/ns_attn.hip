@@ -659,7 +659,9 @@ __device__ __forceinline__ void dma16_run(const uint8_t *base, const uint32_t *o
             : "memory", "m0");
 }
 
-// l plus the sum of a lane's 16 P values as they enter the product, in fp32, two a step.
+// l plus the sum of a lane's 16 P values as they enter the product, in fp32, two a step.  The dot product takes fp16's
+// subnormals as they are (16,384 sums of them were exact); of 49,152 sums of other sizes 4.5% were not the nearest fp32, the
+// worst off by 1.5 units in the last place, and chains of 4,096 by 5e-6 at most.
 __device__ __forceinline__ float add_halves(const half8_t (&p)[2], float l) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)

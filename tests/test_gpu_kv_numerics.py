@@ -1,5 +1,5 @@
 """GPU tests of where attention's arithmetic could go wrong, against the 64-bit oracle with scores that fp32 holds exactly:
-scores of any size, and of minus infinity."""
+scores of any size, scores of minus infinity, weights far below a row's largest, and the few-row kernel's long parts."""
 import math
 
 import pytest
@@ -115,3 +115,77 @@ def test_parts_that_see_only_minus_infinity(ctx, tiles, mid, prefix):
     v = s.v.double()[pages, :, slot // 8, :, slot % 8]  # [keys][kv heads][D]
     ref = v.mean(0).repeat_interleave(2, 0)[None].expand(s.T, 4, D)
     assert_within(got, ref, (2 * O.U16 + 2.0 ** -14) * v.abs().mean(0).repeat_interleave(2, 0)[None] + 2.0 ** -24)
+
+
+@pytest.mark.parametrize("mid", [0, 1], ids=["128", "32"])
+@pytest.mark.parametrize("below", [12.0, 22.6, 23.1, 24.0])
+@pytest.mark.parametrize("dtype", [F16, E4M3], ids=["f16", "e4m3"])
+def test_long_flat_tail_below_one_peak(ctx, tiles, dtype, below, mid):
+    """One key at score 0 and 131,071 whose weights are 2^-below of its own: with fp16 outputs and more than 16 rows P is one
+    fp16, subnormal from 2^-23 on, and has to count in the row's sum as it does in the product."""
+    D, page, kv = 64, 64, 131072
+    s = Setup(dtype, D, 4, 1, page, [(5, kv)], seed=240)
+    k = torch.zeros(s.k.shape)
+    k[:, :, 0, :, 0] = -16.0
+    pg, slot = int(s.table[0, 0]), 5
+    k[pg, :, 0, slot, 0] = 0.0
+    s.k = k.to(dtype)
+    q = torch.zeros(s.rows, 4, D)
+    q[..., 0] = 1.0
+    q = q.half()
+    scale = below * math.log(2) / (16.0 * s.ks)
+    tiles(mid, 1)
+    sums = kv * O.U32  # a lane adds half the row's keys two at a time, a step off by a unit at most, the product 16 at a time
+    # all values equal: whatever the weights are, their sum has to be the products'
+    v = torch.ones(s.v.shape) / s.vs
+    s.v = v.to(dtype)
+    s.device()
+    got = attend(ctx, s, q, scale, True).double().cpu()
+    assert_within(got, torch.ones_like(got), torch.full_like(got, sums + 2.0 ** -20 + O.U16 + 2.0 ** -24))
+    # the peak's value zero: the tail's share, P within half a step of fp16 (2^-25 of its subnormals; the peak is 2^9)
+    v[pg, :, slot // O.CHUNK[dtype], :, slot % O.CHUNK[dtype]] = 0
+    s.v = v.to(dtype)
+    s.device()
+    got = attend(ctx, s, q, scale, True).double().cpu()
+    tail = (kv - torch.arange(5, 0, -1)).double() * 2.0 ** -below  # keys that row i sees but the peak
+    ref = (tail / (1 + tail))[:, None, None].expand(5, 4, D)
+    half_step = max(O.U16, 2.0 ** -25 / 2.0 ** (9.0 - below))
+    assert_within(got, ref, ref * (2 * sums + 2.0 ** -20 + 2 * half_step + O.U16 + 8 * O.U32 * below) + 2.0 ** -25)
+
+
+LONG = [  # dtype, D, q heads, kv heads, page, lengths, window
+    (F16, 64, 8, 8, 64, [(1, 20001)], 0),
+    (F16, 64, 8, 8, 16, [(1, 20000)], 0),
+    (F16, 256, 16, 8, 64, [(1, 12345)], 0),
+    (F16, 128, 16, 8, 256, [(2, 15000)], 12000),
+    (F16, 64, 8, 8, 16, [(1, 26000)], 25000),
+    (E4M3, 64, 16, 8, 64, [(1, 40000)], 0),
+    (E4M3, 64, 16, 8, 16, [(2, 35001)], 0),
+    (E4M3, 128, 8, 8, 32, [(1, 24000)], 20000),
+    (E4M3, 256, 8, 8, 128, [(1, 20000)], 0),
+    (F16, 64, 8, 8, 32, [(1, 30000), (1, 5), (2, 9000), (0, 7), (1, 300)], 0),
+    (E4M3, 64, 8, 8, 64, [(1, 9000), (1, 33000)], 0),
+    (F16, 256, 16, 1, 64, [(1, 6000)], 0),   # 16 rows over 47 parts: the join takes them in three rounds
+    (E4M3, 256, 8, 1, 64, [(2, 11000)], 0),
+]
+
+
+@pytest.mark.parametrize("half_out", [True, False], ids=["f16", "f32"])
+@pytest.mark.parametrize("case", range(len(LONG)))
+def test_long_sequences_of_few_rows(ctx, case, half_out):
+    """Parts of more than four key tiles (a wave takes several, its maximum running over them) and joins of more parts
+    than a round takes, with keys of far larger scores late, in the middle or early."""
+    dtype, D, qh, kh, page, lengths, window = LONG[case]
+    at = (0.97, 0.5, 0.3)[(case + half_out) % 3]  # a window's start lies below all of them
+    s = Setup(dtype, D, qh, kh, page, lengths, seed=260 + case)
+    for i, (_, kv) in enumerate(lengths):
+        p = int(at * (kv - 1))
+        pg, slot = int(s.table[i, p // page]), p % page
+        row = (s.k[pg, :, :, slot].float() * 4).clamp(-448 if dtype == E4M3 else -65504, 448 if dtype == E4M3 else 65504)
+        O.raw(s.k)[pg, :, :, slot] = O.raw(row.to(dtype))  # one key of scores some 4 times the others'
+    s.device()
+    q = s.queries()
+    got = s.attend(ctx, q.cuda(), window, half_out)
+    torch.cuda.synchronize()
+    ref, bound = O.attention(q[:s.T], s.k, s.v, s.table, s.lengths, page, D ** -0.5, window, s.ks, s.vs, half_out, one_p=False)
+    assert_within(got, ref, bound)
