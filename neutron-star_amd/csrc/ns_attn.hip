@@ -625,13 +625,6 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(AttnArgs a) {
     attn_rows<D, E4M3, UNI, STREAM, true>(a, blockIdx.x);
 }
 
-// s_waitcnt vmcnt(N) (gfx9 encoding: vmcnt bits 3:0 and 15:14; expcnt and lgkmcnt left at their largest).
-template <int N>
-__device__ __forceinline__ void vm_wait() {
-    static_assert(N >= 0 && N < 64, "vmcnt is 6 bits");
-    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
-}
-
 // A direct load of 16 bytes per lane into the 1 KiB of LDS at byte `lds`.  The builtin for it makes the compiler wait
 // for every such load before it reads any LDS that it cannot tell apart, so the next tile's loads would never
 // overlap this one's products; here the kernel's own waits order them.  (No destination registers; m0 needs a
@@ -973,13 +966,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_mid_kernel(AttnArg
 // Bound by the matrix pipe and what two waves a SIMD hide of the rest: 2,048 tokens at 32,768 keys, 16 heads on 8 of
 // 256 dims, 1,010 us with the join's 14 (1,050 TFLOP/s; pipe busy 57%, L2 hits 96%).  With 128 dims e4m3, 12 prompts
 // and a window of 1,500, by the vector ALU (10 instructions a matrix one): 205 us, 740 TFLOP/s.
-template <int D, bool E4M3, int NW, int NS, bool HILO, bool PREFIX>
+constexpr int kTileWaves = 4, kTileBuffers = 2;
+constexpr uint32_t kTileRows = 32 * kTileWaves, kMidRows = 32;
+
+template <int D, bool E4M3, bool HILO, bool PREFIX>
 __device__ __forceinline__ void attn_tile(const AttnArgs &a, uint32_t block, uint32_t n_parts) {
-    constexpr int C = E4M3 ? 16 : 8, U = C / 8, KT = 32, TM = 32 * NW;
+    constexpr int C = E4M3 ? 16 : 8, U = C / 8, KT = 32, NW = kTileWaves, NS = kTileBuffers, TM = kTileRows;
     constexpr int KS = D / 16;          // k steps of the first product
     constexpr int DT = D / 32;          // 32-dim tiles of the second
     constexpr int BYTES = KT * D * 16 / C;  // of a K or V tile
-    constexpr int PER = (BYTES / 1024 + NW - 1) / NW * 2;  // direct loads of a wave for a tile, at most
     uint8_t(&kt)[NS][BYTES] = *reinterpret_cast<uint8_t(*)[NS][BYTES]>(smem);
     uint8_t(&vt)[NS][BYTES] = *reinterpret_cast<uint8_t(*)[NS][BYTES]>(smem + NS * BYTES);
     const uint32_t kt_at = uint32_t(uintptr_t((__attribute__((address_space(3))) uint8_t *)smem)), vt_at = kt_at + NS * BYTES;
@@ -1079,26 +1074,26 @@ __device__ __forceinline__ void attn_tile(const AttnArgs &a, uint32_t block, uin
         }
     };
 
-    // Tiles first .. first + NS - 2 are on their way before the loop; each step asks for the one NS - 1 ahead.
+    // The first tile is on its way before the loop; each step asks for the next one.  (A loop of one round: without it
+    // the 256-dim e4m3 instance spills, 238 -> 265 us for 3 x 1,024 tokens of 9,000 keys on pages of 16.)
     auto fetch_tile = [&](uint32_t tile, uint32_t buf) { fetch(tile, page_of(tile * KT), page_of(tile * KT + 16), buf); };
 #pragma unroll
     for (uint32_t i = 0; i < NS - 1; ++i)
         if (first + i < end) fetch_tile(first + i, i);
-    uint32_t pa = page_of((first + NS - 1) * KT), pb = page_of((first + NS - 1) * KT + 16);
+    uint32_t pa = page_of((first + 1) * KT), pb = page_of((first + 1) * KT + 16);
     const uint32_t krow = E4M3 ? 16 * ((col / 4) % 2) + 4 * (col / 8) + col % 4 : 16 * (col / 16) + 8 * ((col / 4) % 2) + 4 * ((col / 8) % 2) + col % 4;
     uint32_t buf = 0;
-    for (uint32_t tile = first; tile < end; ++tile, buf = buf + 1 == NS ? 0 : buf + 1) {
-        // This tile has landed for every wave (loads return in order: those of the NS - 2 tiles behind it may be
-        // out, at the end none is), and every wave is done with the buffer that the next loads go to.
+    for (uint32_t tile = first; tile < end; ++tile, buf ^= 1) {
+        // This tile has landed for every wave, and every wave is done with the buffer that the next loads go to (its
+        // reads of it have returned).
         __atomic_signal_fence(__ATOMIC_SEQ_CST);
-        if (NS > 2 && BYTES / 1024 % NW == 0 && tile + NS - 2 < end) vm_wait<PER *(NS - 2)>();
-        else vm_wait<0>();
+        __builtin_amdgcn_s_waitcnt(0);
         __builtin_amdgcn_s_barrier();
         __atomic_signal_fence(__ATOMIC_SEQ_CST);
-        if (tile + NS - 1 < end) {
-            fetch(tile + NS - 1, pa, pb, buf == 0 ? NS - 1 : buf - 1);
-            pa = page_of((tile + NS) * KT);
-            pb = page_of((tile + NS) * KT + 16);
+        if (tile + 1 < end) {
+            fetch(tile + 1, pa, pb, buf ^ 1);
+            pa = page_of((tile + 2) * KT);
+            pb = page_of((tile + 2) * KT + 16);
         }
         const uint32_t t0 = tile * KT;
         if (t0 < lo || t0 + KT > hi) {  // V outside [lo, hi) may hold anything, and 0 * NaN would reach the sums
@@ -1204,26 +1199,26 @@ __device__ __forceinline__ void attn_tile(const AttnArgs &a, uint32_t block, uin
         }
     if (!whole && hl == 0) *reinterpret_cast<float2 *>(a.stats + 2 * at) = float2{m, l * kUnbias<HILO>};
 }
-template <int D, bool E4M3, int NW, int NS>
+template <int D, bool E4M3>
 struct TileLds {
-    static constexpr uint32_t kBytes = 2 * NS * 32 * D * (E4M3 ? 1 : 2);
+    static constexpr uint32_t kBytes = 2 * kTileBuffers * 32 * D * (E4M3 ? 1 : 2);
 };
-template <int D, bool E4M3, int NW, int NS, bool HILO, bool PREFIX>
-__global__ __launch_bounds__(64 * NW, 2) void attn_tile_kernel(AttnArgs a) {
-    attn_tile<D, E4M3, NW, NS, HILO, PREFIX>(a, blockIdx.x, PREFIX ? a.pre_parts : a.parts);
+template <int D, bool E4M3, bool HILO, bool PREFIX>
+__global__ __launch_bounds__(64 * kTileWaves, 2) void attn_tile_kernel(AttnArgs a) {
+    attn_tile<D, E4M3, HILO, PREFIX>(a, blockIdx.x, PREFIX ? a.pre_parts : a.parts);
 }
 
 // ---- a shared prefix and few rows of each sequence: both kinds of work in one launch --------------------------
 //
-// The prefix's row tiles (all sequences' rows, TR of them a tile) and the sequences' own keys read different
+// The prefix's row tiles (all sequences' rows, MID: 32 of them a tile, otherwise 128) and the sequences' own keys read different
 // memory and do not depend on each other: side by side they keep the memory busy through each other's starts
 // and ends (64 sequences of up to 500 keys of their own on 32,768 tokens, 256 dims, 8 key heads: 70 and 46 us one after
 // the other, 92 side by side: 4.6 TB/s).  Bound by the bytes of the prefix, read once.
-template <int D, bool E4M3, bool UNI, bool HILO, int TR>
-__global__ __launch_bounds__(256, D == 256 && TR == 32 ? 1 : 2) void attn_shared_kernel(AttnArgs a, uint32_t pre_blocks) {
+template <int D, bool E4M3, bool UNI, bool HILO, bool MID>
+__global__ __launch_bounds__(256, D == 256 && MID ? 1 : 2) void attn_shared_kernel(AttnArgs a, uint32_t pre_blocks) {
     if (blockIdx.x < pre_blocks) {
-        if constexpr (TR == 32) attn_mid<D, E4M3, UNI, HILO, true>(a, blockIdx.x, a.pre_parts);
-        else attn_tile<D, E4M3, TR / 32, 2, HILO, true>(a, blockIdx.x, a.pre_parts);
+        if constexpr (MID) attn_mid<D, E4M3, UNI, HILO, true>(a, blockIdx.x, a.pre_parts);
+        else attn_tile<D, E4M3, HILO, true>(a, blockIdx.x, a.pre_parts);
     } else {
         attn_rows<D, E4M3, UNI, false, false>(a, blockIdx.x - pre_blocks);
     }
@@ -1270,9 +1265,6 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
         join_row<D>(a, ps, r, d, q.q0 + row / a.group, head * a.group + row % a.group);
     }
 }
-
-constexpr int kTileWaves = 4, kTileStages = 2;
-constexpr uint32_t kTileRows = 32 * kTileWaves, kMidRows = 32;
 
 // Estimated time (us) of row tiles of `rows` rows: `busy` of them (key heads counted), with `tiles` key tiles at most
 // and `mean` on the average, in p key parts.  kTile and kMid: a key tile's time with 1, 2, ... workgroups on each CU, up
@@ -1384,9 +1376,9 @@ hipError_t launch_tiles(uint32_t rows, uint32_t wgs, const AttnArgs &a, hipStrea
     const dim3 g(wgs), b(256);
     const bool uni = a.kv.page_shift >= 5;
     if (rows == kTileRows) {
-        constexpr uint32_t lds = TileLds<D, E4M3, kTileWaves, kTileStages>::kBytes;
-        if (a.half_out) attn_tile_kernel<D, E4M3, kTileWaves, kTileStages, false, PREFIX><<<g, b, lds, stream>>>(a);
-        else attn_tile_kernel<D, E4M3, kTileWaves, kTileStages, true, PREFIX><<<g, b, lds, stream>>>(a);
+        constexpr uint32_t lds = TileLds<D, E4M3>::kBytes;
+        if (a.half_out) attn_tile_kernel<D, E4M3, false, PREFIX><<<g, b, lds, stream>>>(a);
+        else attn_tile_kernel<D, E4M3, true, PREFIX><<<g, b, lds, stream>>>(a);
     } else {
         constexpr uint32_t lds = MidLds<D>::kBytes;
         if (uni && a.half_out) attn_mid_kernel<D, E4M3, true, false, PREFIX><<<g, b, lds, stream>>>(a);
@@ -1403,9 +1395,9 @@ hipError_t launch_shared(const AttnPlan &p, const AttnArgs &a, hipStream_t strea
     const uint32_t pre = p.pre_tiles * p.pre_parts * a.kv.kv_heads, rows = RowsLds<D>::bytes(p.row_cap);
     const dim3 g(pre + p.row_slots * a.kv.kv_heads), b(256);
     if (p.pre_tile_rows == kTileRows)
-        attn_shared_kernel<D, E4M3, UNI, HILO, kTileRows><<<g, b, std::max(rows, TileLds<D, E4M3, kTileWaves, 2>::kBytes), stream>>>(a, pre);
+        attn_shared_kernel<D, E4M3, UNI, HILO, false><<<g, b, std::max(rows, TileLds<D, E4M3>::kBytes), stream>>>(a, pre);
     else
-        attn_shared_kernel<D, E4M3, UNI, HILO, kMidRows><<<g, b, std::max(rows, MidLds<D>::kBytes), stream>>>(a, pre);
+        attn_shared_kernel<D, E4M3, UNI, HILO, true><<<g, b, std::max(rows, MidLds<D>::kBytes), stream>>>(a, pre);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     const uint32_t per = 256 / (D / 4);
     attn_shared_join_kernel<D><<<dim3((a.kv.tokens * a.group + per - 1) / per * a.kv.kv_heads), b, 0, stream>>>(a);
