@@ -747,12 +747,14 @@ int append(ns_ctx *ctx, const char *fn, const ns_kv_cache *cache, const ns_kv_ba
     return e == hipSuccess ? NS_OK : hip_fail(e, fn);
 }
 
-// No C++ exception leaves a C entry (the host's memory may run out while a message or a retired buffer is noted).
+// No C++ exception leaves a C entry (the host's memory may run out while a message or a retired buffer is noted).  The
+// message is short enough for a string's own room, so noting it allocates nothing.
 template <class F>
 int no_throw(F &&f) {
     try {
         return f();
     } catch (...) {
+        set_error("no host memory");
         return NS_ERR_HIP;
     }
 }
