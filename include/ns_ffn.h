@@ -299,8 +299,8 @@ int ns_qkv(ns_ctx *ctx, const void *wq, const void *wk, const void *wv, int v_ty
  * graph runs again on new contents of the same buffers.  The host's numbers (max_q, max_kv, tokens,
  * seqs) are bounds that the launches are planned for. */
 
-/* Element types of a cache.  E4M3: 8-bit floats of 4 exponent and 3 mantissa bits (largest 448,
- * no infinities), round to nearest even; values past the range saturate, NaN stays NaN. */
+/* Element types of a cache, rounded to nearest even.  F16: values past its range become infinities.  E4M3: 8-bit
+ * floats of 4 exponent and 3 mantissa bits (largest 448, no infinities); values past the range saturate, NaN stays NaN. */
 enum { NS_KV_F16 = 0, NS_KV_E4M3 = 1 };
 /* The pairs that the rotation turns: (i, i + rot/2), or (2i, 2i + 1). */
 enum { NS_ROPE_HALVES = 0, NS_ROPE_PAIRS = 1 };
@@ -355,8 +355,10 @@ int ns_kv_append(ns_ctx *ctx, const ns_kv_cache *cache, const ns_kv_batch *batch
  * (causal) and, with window > 0, the last `window` of them, its own included.  q fp16 bits
  * [tokens][q_heads][head_dim]; query head h reads key/value head h / (q_heads / kv_heads) (q_heads a
  * multiple of kv_heads).  out fp16 bits (half_out) or fp32, [tokens][q_heads][head_dim].  scale positive
- * and finite.  Scores, statistics and sums are fp32; the softmax weights enter the second product as one
- * fp16 of 11 bits (half_out, above 16 rows of a sequence and key/value head) or as a sum of two.  A NaN
+ * and finite, its product with k_scale between 1e-30 and 1e30.  Scores, statistics and sums are fp32, scores of any
+ * size (only their differences count).  The softmax weights enter the second product as a sum of two fp16 (22 bits),
+ * or with half_out as one of 11 bits for sequences of more than 16 rows a key/value head, and against a shared prefix
+ * for all: an error like that of the output's own rounding (a caller who wants less takes fp32 out).  A NaN
  * or infinity in a token's value reaches the rows that see it and may reach other rows of the same
  * sequence, never another sequence's; what a cache holds outside the sequences' positions, and before
  * every row's window, is without effect whatever it is.

@@ -35,7 +35,9 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // creeps up.  P <= 2^(bias + lag) has to stay below fp16's 65504.  As two fp16 P keeps 22 bits down to 2^-28 of the
 // maximum, and what falls below is less than fp32's own rounding over any number of keys that fits the cache;
 // as one it keeps its 11 bits down to 2^-22, and 2^18 keys below 2^-33 come to 2^-15 of the sum, against 2^-11 of
-// the output's own rounding.
+// the output's own rounding.  One fp16 is taken by the row tiles of fp16 outputs, those of a shared prefix among them, also
+// where each sequence has few rows of its own: as two, 64 sequences on a prefix of 32,768 take 135 us instead of 107
+// (128-dim heads, 4 tokens each: 207 instead of 159).
 template <bool HILO>
 constexpr float kBias = HILO ? 14.0f : 9.0f;
 template <bool HILO>
@@ -47,7 +49,8 @@ constexpr float kUnbias = HILO ? 0x1p-14f : 0x1p-9f;  // parts are kept without 
 // formed first, exact for the scores that weigh: a wave with such a row, or with one that has seen nothing yet (m = -inf, its
 // scores as well: 0 is subtracted), takes the branch of a raised maximum for every tile.  Parts are compared by m
 // itself for the same reason.  (2,048 tokens at 32,768 keys 1,028 -> 1,034 us, 157 tokens 22.4 -> 22.7, against always the
-// one operation.)
+// one operation.)  The step stands in each kernel: as a function over their scores and O it takes 10 to 20 registers
+// more, and the 256-dim instances spill 60 bytes a lane and more.
 constexpr float kFar = 1024.0f;
 // The |m| from which a row is far.  Formed in the kernel: a launch argument more costs each of them some .2 us.
 __device__ __forceinline__ float far_max(float c1) {
@@ -291,7 +294,8 @@ __device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane) { return ui
 // group g = l / 16.  Row m of K row tile t is key c (m / 4) + 4 t + m % 4, so lane l's scores are those of
 // keys c g ... c g + c - 1, the chunk of V that it reads.  The next tile's K loads are issued before
 // the softmax of this one.  Bound by the bytes of K and V: fp16, 256 dims, 8 key heads, one token at 262,144 keys
-// 319 us (6.7 TB/s), 32 sequences up to 8,192 keys 197 us (5.6 TB/s).  Short calls are bound by a chain of
+// 319-336 us a call on different boxes (6.4-6.7 TB/s; 320 us the shortest launch in a trace of the 319 us one), 32
+// sequences up to 8,192 keys 197 us (5.6 TB/s).  Short calls are bound by a chain of
 // dependent steps: one token at 2,206 keys 9.2 us, of which 2.5 until the first K is asked for (lengths, scan over the
 // sequences, table entry), 1.8 for loads and products, .9 to join the waves, 1.8 for the parts' way to memory and
 // the count, 2.2 for the join.
@@ -304,7 +308,8 @@ struct RowsLds {
                               kFixed = kStats + 16;
     static constexpr uint32_t bytes(uint32_t row_cap) { return kFixed + 4 * row_cap * (D + 4) * 4; }
 };
-// STREAM: K and V are loaded as data that is not used again, which a single sequence's are (262,144 keys: 374 -> 336 us).
+// STREAM: K and V are loaded as data that is not used again, which a single sequence's are (262,144 keys: 374 -> 336 us on
+// one box, 360 -> 319 on another).
 // Sequences may share pages, and find each other's in the caches (64 of them on a prefix of 32,768: 756 us, 1,787
 // with such loads).
 template <int D, bool E4M3, bool UNI, bool STREAM, bool JOIN>
@@ -715,7 +720,7 @@ __device__ __forceinline__ bool tile_span(const AttnArgs &a, uint32_t slot, uint
 // For calls whose row tiles of 128 are too few to fill the chip: the keys are split four ways without parts in
 // memory.  A wave of 256 dims holds 128 O, 128 K and V registers: one workgroup a CU.  Bound by the latency of its
 // loads: 157 tokens on 2,205 keys, 16 heads on 8 of 256 dims, 17 us and 4 for the join (32 in row tiles of
-// 128); the matrix pipe is busy 17% of the time.
+// 128); the matrix pipe is busy 16% of the time.
 template <int D>
 struct MidLds {
     static constexpr uint32_t kQueries = 32 * (D + 8) * 2, kFixed = kQueries + 2 * 4 * 32 * 4, kBytes = kFixed + 4 * 32 * (D + 4) * 4;
@@ -1268,11 +1273,13 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 
 // Estimated time (us) of row tiles of `rows` rows: `busy` of them (key heads counted), with `tiles` key tiles at most
 // and `mean` on the average, in p key parts.  kTile and kMid: a key tile's time with 1, 2, ... workgroups on each CU, up
-// to as many as fit (one sequence of 8 key heads, 2,048 and 8,192 keys before 1,024 to 16,384 rows).  The
-// longest start first, so the time is the longest workgroup's, or all of them through the slots of the chip with
-// half of one at the end.  The other constants are fitted to 450 calls of 17 to 5,800 tokens a sequence and up to
-// 40,000 keys; on 500 more the choice took 1.03 times the fastest of all choices on the average, and at most 1.12
-// times in nine of ten (most of the others: batches far shorter than their bounds say).
+// to as many as fit (one sequence of 8 key heads, 2,048 and 8,192 keys before 1,024 to 16,384 rows; fp16 outputs of
+// an fp16 cache: e4m3 caches and fp32 outputs go by the same figures, though the 128-dim instances of fp32 outputs
+// have registers for two workgroups a CU, not three).  The longest start first, so the time is the longest workgroup's,
+// or all of them through the slots of the chip with half of one at the end.  The other constants are fitted to 450
+// calls of 17 to 5,800 tokens a sequence and up to 40,000 keys; on 300 others, of all types and outputs, the choice took
+// 1.03 times the fastest of all choices on the average, at most 1.09 times in nine of ten and 1.17 in 97 of 100 (most of
+// the others: batches far shorter than their bounds say).
 struct TileWork {
     uint32_t head_dim, busy, tiles;
     double mean;
@@ -1324,6 +1331,9 @@ AttnPlan plan_attn(const AttnShape &s, const Tuning &tune) {
         // full on the average, so parts of total / target tiles are target + seqs / 2 in number.
         const uint32_t round = std::max(1u, 2 * cus / s.kv_heads), rounds = (s.seqs + round - 1) / round;
         p.target = std::min(kPartsMax / 2, std::max(1u, rounds * round - s.seqs / 2));
+        // A part is four tiles or more, one for each wave.  Calls in us with 1 / 2 / 4 / 8 / 32: one token at 2,206 keys 13.4 /
+        // 13.5 / 11.3 / 12.6 / 26, at 700 keys 10.4 / 9.4 / 10.2 / 12.8 / 19, three in a window of 1,024 (e4m3) 14.7 / 11.6 / 11.6 /
+        // 13.6 / 16.5, 8 sequences up to 1,500 keys (e4m3) 10.8 / 10.9 / 10.6 / 11.0 / 12.7.  (32: the short ones without a join.)
         p.min_tiles = 4;
         const uint64_t most = uint64_t(s.seqs) * ((keys / kt + 2 + p.min_tiles - 1) / p.min_tiles);
         p.row_slots = uint32_t(std::min<uint64_t>(most, uint64_t(p.target) + s.seqs));
