@@ -12,29 +12,30 @@ from test_gpu_kv_attention import E4M3, F16, Setup, assert_within, ctx, tiles  #
 pytestmark = pytest.mark.gpu
 
 
-def exact_scores(s, q, scale, half_out, one_p):
+def exact_scores(s, q, scale, half_out, one_p, window=0):
     """(out, bound) where every score q.k is exact in fp32 and a row's scores are equal or far apart, so that no error of
     the scores counts: P's rounding, fp32 sums of kv terms, the output's rounding."""
     out, bound = torch.zeros(s.T, s.qh, s.D, dtype=torch.float64), torch.zeros(s.T, s.qh, s.D, dtype=torch.float64)
     t = 0
-    for i, (n, kv) in enumerate(s.lengths):
-        k = O.sequence(s.k, s.table[i], s.page, kv, s.ks, False).repeat_interleave(s.qh // s.kh, 0)
-        v = O.sequence(s.v, s.table[i], s.page, kv, s.vs, True).repeat_interleave(s.qh // s.kh, 0)
+    for b, (n, kv) in enumerate(s.lengths):
+        k = O.sequence(s.k, s.table[b], s.page, kv, s.ks, False).repeat_interleave(s.qh // s.kh, 0)
+        v = O.sequence(s.v, s.table[b], s.page, kv, s.vs, True).repeat_interleave(s.qh // s.kh, 0)
         x = q[t:t + n].double().transpose(0, 1) @ k.transpose(1, 2) * scale
-        x = x.masked_fill(torch.arange(kv)[None] > torch.arange(kv - n, kv)[:, None], -math.inf)
+        i, j = torch.arange(kv - n, kv)[:, None], torch.arange(kv)[None]
+        x = x.masked_fill((j > i) | (j <= i - (window or kv)), -math.inf)
         p = torch.softmax(x, -1)
         o = p @ v
-        b = ((kv + 64) * O.U32 + 2.0 ** -20 + (O.U16 if one_p else 0.0)) * (p @ v.abs())
-        b = b + (O.U16 * o.abs() + 2.0 ** -24 if half_out else 2 * O.U32 * o.abs())
-        out[t:t + n], bound[t:t + n] = o.transpose(0, 1), b.transpose(0, 1)
+        err = ((kv + 64) * O.U32 + 2.0 ** -20 + (O.U16 if one_p else 0.0)) * (p @ v.abs())
+        err = err + (O.U16 * o.abs() + 2.0 ** -24 if half_out else 2 * O.U32 * o.abs())
+        out[t:t + n], bound[t:t + n] = o.transpose(0, 1), err.transpose(0, 1)
         t += n
     return out, bound
 
 
-def attend(ctx, s, q, scale, half_out, prefix=None):
+def attend(ctx, s, q, scale, half_out, prefix=None, window=0):
     out = torch.full((s.rows, s.qh, s.D), 7.0, dtype=F16 if half_out else torch.float32, device="cuda")
     if prefix is None:
-        ctx.paged_attention(s.cache, s.batch, q.cuda(), s.qh, scale, out, half_out=half_out)
+        ctx.paged_attention(s.cache, s.batch, q.cuda(), s.qh, scale, out, window=window, half_out=half_out)
     else:
         ctx.shared_prefix_attention(s.cache, s.batch, prefix, q.cuda(), s.qh, scale, out, half_out=half_out)
     torch.cuda.synchronize()
@@ -88,6 +89,30 @@ def test_scores_of_any_size(ctx, tiles, case, top, half_out):
         assert_within(got, ref, bound + slack * float(s.vs * s.v.float().abs().max()))
         if s.max_q * (qh // kh) <= 16 and prefix is None:
             break
+
+
+@pytest.mark.parametrize("half_out", [True, False], ids=["f16", "f32"])
+@pytest.mark.parametrize("window", [1, 33, 100])
+@pytest.mark.parametrize("lengths", [[(1, 300), (4, 90), (2, 2)], [(150, 400), (40, 40), (3, 70)]], ids=["few-rows", "tiles"])
+def test_large_scores_in_a_window(ctx, tiles, lengths, window, half_out):
+    """The same where rows of a tile have seen nothing yet beside rows of large scores, and beside rows of scores 0."""
+    s = Setup(F16, 64, 8, 2, 16, lengths, seed=225, fill=math.nan)
+    k = s.k.float()
+    held = torch.isfinite(k)
+    k[held] = 0
+    level = torch.tensor([256.0, 128.0, -256.0])[torch.randint(0, 3, k[:, :, 0, :, 0].shape, generator=s.gen)]
+    k[:, :, 0, :, 0] = torch.where(held[:, :, 0, :, 0], level, k[:, :, 0, :, 0])
+    s.k = k.half()
+    s.device()
+    q = torch.zeros(s.rows, 8, 64)
+    q[..., 0] = torch.randint(1024, 2048, (s.rows, 8), generator=s.gen) * torch.randint(-1, 2, (s.rows, 8), generator=s.gen)
+    q = q.half()
+    for top in (1e5, 1e9):
+        for mid, parts in ((-1, 0), (0, 1), (0, 4), (1, 1), (1, 4)):
+            tiles(mid, parts)
+            got = attend(ctx, s, q, top / (2047 * 256), half_out, window=window)
+            ref, bound = exact_scores(s, q, top / (2047 * 256), half_out, half_out, window)
+            assert_within(got, ref, bound)
 
 
 @pytest.mark.parametrize("mid", [0, 1], ids=["128", "32"])
