@@ -40,7 +40,10 @@ int fail(int code, const std::string &msg) {
     return code;
 }
 
+// The runtime keeps a failed call's error until it is asked for: reported here, it is not left for the caller's next
+// call (of this library or any other) to find.
 int hip_fail(hipError_t e, const char *what) {
+    (void)hipGetLastError();
     return fail(NS_ERR_HIP, std::string(what) + ": " + hipGetErrorString(e));
 }
 

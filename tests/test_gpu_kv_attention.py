@@ -580,6 +580,29 @@ def test_two_graphs_and_a_grown_workspace():
     c.close()
 
 
+def test_a_refused_workspace_leaves_the_next_call_alone():
+    """A call whose parts would need more memory than the card has (over a tebibyte) returns an error and runs nothing;
+    the next call is as ever."""
+    c = N.Context(0)
+    s = Setup(F16, 256, 16, 8, 64, [(1, 300), (1, 200)], seed=120, shared=2)
+    q = s.queries().cuda()
+    ref, bound = s.expect(q.cpu())
+    c.set_tuning("attn_mid", 0)
+    c.set_tuning("attn_parts", 32)
+    many = N.KvBatch(s.dtable, s.dstarts, s.dlen, 1 << 21, 1, s.max_kv)  # 2^25 rows, in 32 parts of 1 KiB each
+    assert (1 << 25) * 32 * 1024 > 2 * torch.cuda.mem_get_info()[1]
+    big = [torch.empty(1 << 21, 16, 256, dtype=F16, device="cuda") for _ in range(2)]
+    with pytest.raises(N.NsError, match="memory"):
+        c.shared_prefix_attention(s.cache, many, 2, big[0], 16, 1 / 16, big[1])
+    del big
+    torch.cuda.empty_cache()
+    c.set_tuning("attn_mid", -1)
+    c.set_tuning("attn_parts", 0)
+    assert_within(s.attend(c, q, prefix=2), ref, bound)
+    torch.cuda.synchronize()
+    c.close()
+
+
 def test_on_another_stream(ctx):
     s = Setup(F16, 256, 16, 8, 64, [(1, 3000), (20, 200)], seed=102)
     q = s.queries()
